@@ -102,20 +102,25 @@ __device__ __forceinline__ void paged_store_quad(uint8_t* group, int which, int 
 }
 
 // Up to 16 rows from r0 on: how many there are, and whether they are consecutive positions of one
-// sequence (of which the first is then `pos` of `seq`). All lanes of the warp call it.
+// sequence that its row of the page table reaches (of which the first is then `pos` of `seq`): what
+// lies beyond goes row by row, so that no loop over a run's positions comes near INT_MAX. All lanes
+// of the warp call it.
 struct PagedRun {
     int n, seq, pos;
     bool run;
 };
-__device__ __forceinline__ PagedRun paged_run(const int32_t* pos, const int32_t* seq, int r0, int n_rows) {
+__device__ __forceinline__ PagedRun paged_run(const PagedView& v, const int32_t* pos, const int32_t* seq,
+                                              int r0, int n_rows) {
     const int lane = threadIdx.x & 31;
     PagedRun u;
     u.n = min(16, n_rows - r0);
-    const int r = r0 + min(lane, u.n - 1);
-    const int p = pos[r], q = seq ? seq[r] : r;
+    const int i = min(lane, u.n - 1);
+    const int p = pos[r0 + i], q = seq ? seq[r0 + i] : r0 + i;
     u.pos = __shfl_sync(0xffffffffu, p, 0);
     u.seq = __shfl_sync(0xffffffffu, q, 0);
-    u.run = __all_sync(0xffffffffu, q == u.seq && p == u.pos + min(lane, u.n - 1) && u.pos >= 0);
+    const int last = (v.pages_per_seq << v.page_shift) - u.n;  // at most 2^31 - 1 positions
+    u.run = __all_sync(0xffffffffu, q == u.seq && (uint32_t)p - (uint32_t)u.pos == (uint32_t)i) &&
+            u.pos >= 0 && u.pos <= last;
     return u;
 }
 
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 4 : 3) k_paged_append(const P
     if (blockIdx.x < a.value_ctas) {  // ---- values: 16 rows, 8 heads
         const uint32_t block = blockIdx.x / a.head_ctas;
         const int r0 = (int)block * 16, hv = (int)(blockIdx.x - block * a.head_ctas) * 8;
-        const PagedRun u = paged_run(a.pos, a.seq, r0, a.n_rows);
+        const PagedRun u = paged_run(a.v, a.pos, a.seq, r0, a.n_rows);
         if (u.run) {
             if (hv + warp < a.v.n_head_kv)
                 paged_store_v<TYPE, HD, VEC>(a.v, a.x + (int64_t)r0 * a.x_stride, a.x_stride, hv + warp,
@@ -559,7 +564,7 @@ __global__ void __launch_bounds__(256) k_paged_read(const PagedReadArgs a) {
     const int warp = threadIdx.x >> 5, r0 = blockIdx.x * 16, h0 = blockIdx.y * 8;
     const int nh = min(8, a.v.n_head_kv - h0);
     pdl_wait();
-    const PagedRun u = paged_run(a.pos, a.seq, r0, a.n_rows);
+    const PagedRun u = paged_run(a.v, a.pos, a.seq, r0, a.n_rows);
     auto all = [&](auto out) {
         constexpr int OUT = decltype(out)::value;
         if (!u.run) {

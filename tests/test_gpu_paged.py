@@ -781,3 +781,64 @@ def test_a_run_that_leaves_its_pages_or_the_rotation_table(ctx):
         assert torch.equal(vo.cpu(), want)
         assert not ko[last:].any() and not ko[:start].any() and ko[start:last].any()
     kv.free()
+
+
+@pytest.mark.parametrize("wtype", TYPES)
+@pytest.mark.parametrize("turned", [False, True])
+def test_positions_up_to_the_largest_number(ctx, wtype, turned):
+    """The table's last position, the first one behind it and the largest numbers there are, alone
+    and as runs of 16: what has no page is reported, writes nothing and reads as zeros."""
+    rng = np.random.default_rng(22)
+    page, hk, d, cap, top = 16, 2, 64, 48, 2 ** 31 - 1
+    kv = ssdllm.PagedKvCache(ctx, 3, page, hk, d, wtype)
+    table = i32([[2, 0, 1]])
+    rope = torch.tensor([1.0, 0.0], device=DEV).repeat(64, d // 2, 1) if turned else None
+    zero = torch.zeros(cap, hk * d, device=DEV)
+    x = torch.from_numpy(rng.standard_normal((16, hk * d)).astype(np.float32)).to(DEV)
+    held = torch.from_numpy(stands_for(x.cpu().numpy(), wtype))
+    for first, n in ((cap - 1, 1), (cap, 1), (cap - 16, 16), (cap - 8, 16), (cap, 16), (top - 31, 16), (top - 16, 1),
+                     (top - 15, 1), (top - 15, 16), (top - 7, 4), (top - 1, 2), (top - 1, 1), (top, 1)):
+        kv.append(zero, zero, i32(np.arange(cap)), table, seq=i32([0] * cap))
+        pos, seq = i32(np.arange(first, first + n)), i32([0] * n)
+        qo = torch.full((n, 2 * hk * d), float("nan"), device=DEV)
+        kv.append(x[:n], x[:n], pos, table, seq=seq, q=torch.ones_like(qo), q_out=qo, rope=rope, rope_halves=True)
+        kept = max(0, min(n, cap - first))
+        assert ctx.device_status() == (0 if kept == n else 3)
+        assert (qo[:kept] == 1).all() and (qo[kept:] == 0).all()
+        whole = torch.zeros(cap, hk * d)
+        whole[first:first + kept] = held[:kept]
+        part = torch.cat([held[:kept], torch.zeros(n - kept, hk * d)])
+        for at, want in ((np.arange(cap), whole), (np.arange(first, first + n), part)):
+            o = torch.full((2, len(at), hk * d), float("nan"), device=DEV)
+            kv.read(i32(at), table, o[0], o[1], seq=i32([0] * len(at)))
+            assert torch.equal(o[0].cpu(), want) and torch.equal(o[1].cpu(), want), (first, n)
+    kv.free()
+
+
+@pytest.mark.parametrize("d", [64, 256])
+def test_the_last_pages_of_the_longest_table(ctx, d):
+    """A table of 2^27 - 1 pages of 16 positions, as long as one may be: its last positions."""
+    rng = np.random.default_rng(23)
+    pages, n = 2 ** 27 - 1, 41
+    end = pages * 16
+    kv = ssdllm.PagedKvCache(ctx, 4, 16, 1, d, F16)
+    table = torch.full((1, pages), -1, dtype=torch.int32, device=DEV)
+    table[0, -3:] = i32([3, 0, 2])
+    k, v = rng.standard_normal((2, n, 1, d)).astype(np.float32)
+    pos = torch.arange(end - n, end, device=DEV).to(torch.int32)
+    seq = i32([0] * n)
+    kv.append(torch.from_numpy(k).to(DEV), torch.from_numpy(v).to(DEV), pos, table, seq=seq)
+    assert ctx.device_status() == 0
+    held = [tuple(stands_for(x, F16).astype(np.float64) for x in (k, v))]
+    o = torch.full((2, n, d), float("nan"), device=DEV)
+    kv.read(pos, table, o[0], o[1], seq=seq)
+    for got, want in zip(o, held[0]):
+        assert np.array_equal(got.cpu().numpy(), want.reshape(n, d).astype(np.float32))
+    q = rng.standard_normal((1, 4, d)).astype(np.float32)
+    out = torch.full((1, 4 * d), float("nan"), device=DEV)
+    for window in (1, 30, n):
+        kv.attention(torch.from_numpy(q.reshape(1, -1)).to(DEV), torch.tensor([end], device=DEV).to(torch.int32), table,
+                     out, kv.attention_workspace(), window=window)
+        check_attention(out, q, held, [n], window=window)
+    assert ctx.device_status() == 0
+    kv.free()
