@@ -67,6 +67,10 @@ constexpr float kLazy = 16.0f;
 // smallest number at the lower end).
 constexpr float kLift = 13.0f, kUnlift = 1.0f / 8192.0f;
 constexpr float kSmall = 1.0f / 2048.0f, kSmallLog = -11.0f, kStep = 16777216.0f;
+// Products with q become scores within the subtraction of the tile's largest score, in one rounding;
+// the largest one has a rounding of its own, a sixteenth at 2^20 and without bound above. Where it is
+// larger (2^20 to infinity, as bits of its magnitude), the largest product is subtracted first.
+constexpr uint32_t kLargeFrom = 0x49800000u, kLargeTo = 0x7F800000u;
 
 template <int TYPE, int HD, bool PACK>
 struct PagedCfg {
@@ -866,7 +870,9 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                 }
                 mx *= c1;
                 float base = mx == -INFINITY ? 0.0f : mx - kLift;  // weights are 2^(x c1 - base)
-                bool update = mx > m + kLazy, again = false;
+                const bool large = (__float_as_uint(mx) & 0x7FFFFFFFu) - kLargeFrom < kLargeTo - kLargeFrom;
+                bool update = mx > m + kLazy || large, again = false;
+                float taken = 0.0f;  // what of mx is subtracted from the products already
                 float dm = 0.0f;
                 if constexpr (C::QT) {
                     dm = T[0].v_scale_max();
@@ -910,10 +916,27 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                                 unlift = __uint_as_float((uint32_t)(127 - 13 - k) << 23) * C::CODE;
                             }
                         }
+                        if (__any_sync(0xffffffffu, large)) {
+                            float top = -INFINITY;
+#pragma unroll
+                            for (int j = 0; j < TP; j++)
+                                top = fmaxf(top, fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                            if (top > -INFINITY) {
+                                taken = mx;
+                                base = -kLift;
+#pragma unroll
+                                for (int j = 0; j < TP; j++)
+#pragma unroll
+                                    for (int k = 0; k < 4; k++) x[j][k] -= top;
+                            }
+                            again = NS == 2;
+                        }
                     }
                 }
                 float w[TP][4], fa = 1.0f, fb = 1.0f;  // weights; what P V of heads 2t, 2t+1 counts
-                if constexpr (NS == 3) base = m == -INFINITY ? 0.0f : m;
+                if constexpr (NS == 3) base = m == -INFINITY ? 0.0f : m - taken;
 #pragma unroll
                 for (int j = 0; j < TP; j++)
 #pragma unroll

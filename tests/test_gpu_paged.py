@@ -842,3 +842,35 @@ def test_the_last_pages_of_the_longest_table(ctx, d):
         check_attention(out, q, held, [n], window=window)
     assert ctx.device_status() == 0
     kv.free()
+
+
+@pytest.mark.parametrize("wtype", TYPES)
+@pytest.mark.parametrize("size", [1e6, 1e8, 1e10, 1e20, 1e34])
+@pytest.mark.parametrize("n", [30, 300, 9000])
+def test_large_scores(ctx, wtype, size, n):
+    """Scores far beyond what an f32 number holds to a whole unit: the largest has all the weight;
+    equal ones, positive or negative, share it."""
+    rng = np.random.default_rng(25)
+    d, h, hk, at = 64, 8, 2, n - 7
+    q = ((0.5 + rng.random((1, h, d))) * size).astype(np.float32)
+    v = rng.standard_normal((n, hk, d)).astype(np.float32)
+    vs = stands_for(v, wtype).astype(np.float64)
+    for kind in ("one", "equal", "equal and negative"):
+        k = np.repeat(rng.random((1, hk, d)) + 0.5, n, 0).astype(np.float32) * (-1 if "neg" in kind else 1)
+        if kind == "one":
+            k[:] = rng.standard_normal((n, hk, d)) * 0.05
+            k[at] = 1.0
+        kv = ssdllm.PagedKvCache(ctx, n // 32 + 1, 32, hk, d, wtype)
+        table = make_table(rng, [n], 32, n // 32 + 1)
+        kv.append(torch.from_numpy(k).to(DEV), torch.from_numpy(v).to(DEV), i32(np.arange(n)), i32(table),
+                  seq=i32([0] * n))
+        if kind == "one":
+            s = np.einsum("hgd,phd->hgp", q[0].astype(np.float64).reshape(hk, h // hk, d), stands_for(k, wtype)) / 8
+            assert (s[..., at, None] - np.delete(s, at, -1) > 0.3 * 8 * size).all()  # e^-margin is nothing
+            want = vs[at]
+            bound = 2.0 ** -20 * np.abs(want)
+        else:
+            want, bound = vs.mean(0), 2.0 ** -20 * np.abs(vs).mean(0)
+        got = run_attention(kv, q, [n], table).cpu().numpy().astype(np.float64).reshape(hk, h // hk, d)
+        assert (np.abs(got - want[:, None]) <= bound[:, None]).all(), kind
+        kv.free()
