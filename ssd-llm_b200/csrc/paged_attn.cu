@@ -869,10 +869,10 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 }
                 mx *= c1;
-                float base = mx == -INFINITY ? 0.0f : mx - kLift;  // weights are 2^(x c1 - base)
+                // weights are 2^(x c1 - base): relative to the tile's largest, or to m
+                float base = NS == 3 ? (m == -INFINITY ? 0.0f : m) : (mx == -INFINITY ? 0.0f : mx - kLift);
                 const bool large = (__float_as_uint(mx) & 0x7FFFFFFFu) - kLargeFrom < kLargeTo - kLargeFrom;
                 bool update = mx > m + kLazy || large, again = false;
-                float taken = 0.0f;  // what of mx is subtracted from the products already
                 float dm = 0.0f;
                 if constexpr (C::QT) {
                     dm = T[0].v_scale_max();
@@ -896,6 +896,7 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                         const float mn = fmaxf(m, mx);
                         const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
                         m = mn;
+                        if constexpr (NS == 3) base = m == -INFINITY ? 0.0f : m;
                         l *= f;
                         const float f0 = __shfl_sync(0xffffffffu, f, 8 * t);
                         const float f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
@@ -924,8 +925,7 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                             if (top > -INFINITY) {
-                                taken = mx;
-                                base = -kLift;
+                                base = NS == 3 ? m - mx : -kLift;
 #pragma unroll
                                 for (int j = 0; j < TP; j++)
 #pragma unroll
@@ -936,7 +936,6 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                     }
                 }
                 float w[TP][4], fa = 1.0f, fb = 1.0f;  // weights; what P V of heads 2t, 2t+1 counts
-                if constexpr (NS == 3) base = m == -INFINITY ? 0.0f : m - taken;
 #pragma unroll
                 for (int j = 0; j < TP; j++)
 #pragma unroll
