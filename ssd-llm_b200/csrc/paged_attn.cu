@@ -80,6 +80,9 @@ struct PagedCfg {
     static constexpr int NP = PACK ? (NS + 1) / 2 : NS;      // products of a fragment with them
     static constexpr int HEADS = PACK ? 4 : 8;               // query heads of a unit
     static constexpr int KW = TYPE == SSD_TYPE_Q8_0 ? 4 : (TYPE == SSD_TYPE_Q4_0 ? 2 : 8);  // words a block
+    // Queries are scaled into [2^QLIFT, 2^(QLIFT + 1)): f16 parts as high as their range allows; bf16
+    // parts have f32's range and stay so low that no finite key overflows a sum of 256 products.
+    static constexpr int QLIFT = NS == 3 ? -10 : 13;
     static constexpr float CODE = TYPE == SSD_TYPE_Q8_0 ? 16777216.0f : 1.0f;  // code / fragment
     static constexpr int HALF = paged_half_bytes(TYPE, HD);  // bytes of a group's K, or V
     static constexpr int ROW = HD + 4;                       // floats of a head in a partial
@@ -716,7 +719,7 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
             const PagedRow& rw = cur.w;
             const int tile = cur.tile, r = cur.r, hk = cur.hk, h0 = cur.sub * HEADS;
             const int n = min(rw.tiles - tile, e - s);
-            // ---- q fragments of the unit's heads, head g's scaled into [2^13, 2^14)
+            // ---- q fragments of the unit's heads, head g's scaled into [2^QLIFT, 2^(QLIFT + 1))
             float c1;
             uint32_t qf[C::QSM ? 1 : NB][NP][4];  // step s, register i: 2 s + i
             uint4* qs = reinterpret_cast<uint4*>(qsm) + lane;
@@ -741,9 +744,10 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 int ex = (int)(__float_as_uint(amax) >> 23);
-                ex = ex == 255 ? 127 : max(ex, 14);
-                const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
-                c1 = fmaxf(__uint_as_float((uint32_t)(ex - 13) << 23) * a.scale * kLog2e * C::CODE, FLT_MIN);
+                // (largest queries below 2^-113: less; beside a bf16 cache above 2^60: down by 2^70)
+                ex = ex == 255 ? 127 : min(max(ex, 14), NS == 3 ? 187 : 254);
+                const float up = __uint_as_float((uint32_t)(254 + C::QLIFT - ex) << 23);
+                c1 = fmaxf(__uint_as_float((uint32_t)(ex - C::QLIFT) << 23) * a.scale * kLog2e * C::CODE, FLT_MIN);
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
                     uint32_t(&f)[NP][4] = qf[C::QSM ? 0 : b];

@@ -874,3 +874,31 @@ def test_large_scores(ctx, wtype, size, n):
         got = run_attention(kv, q, [n], table).cpu().numpy().astype(np.float64).reshape(hk, h // hk, d)
         assert (np.abs(got - want[:, None]) <= bound[:, None]).all(), kind
         kv.free()
+
+
+@pytest.mark.parametrize("d,h,hk", [(64, 8, 2), (128, 16, 2), (256, 6, 1)])
+@pytest.mark.parametrize("key,size", [(1e33, 1.0), (1e36, 1.0), (3e38, 1e-3), (3e38, 1e-30), (1e-6, 1e30), (1.0, 1e36)])
+def test_largest_keys_of_a_bf16_cache(ctx, d, h, hk, key, size):
+    """Keys and queries of any size whose scores are f32 numbers: a position far above the others
+    has all the weight, one far below them none."""
+    rng = np.random.default_rng(24)
+    n, at, scale = 300, 211, 0.1
+    q = ((0.5 + rng.random((1, h, d))) * size).astype(np.float32)
+    k = (rng.standard_normal((n, hk, d)) * min(1.0, 1.0 / size)).astype(np.float32)
+    v = rng.standard_normal((n, hk, d)).astype(np.float32)
+    for sign in (1.0, -1.0):
+        kv = ssdllm.PagedKvCache(ctx, 20, 16, hk, d, BF16)
+        table = make_table(rng, [n], 16, 20)
+        k[at] = sign * key
+        kv.append(torch.from_numpy(k).to(DEV), torch.from_numpy(v).to(DEV), i32(np.arange(n)), i32(table),
+                  seq=i32([0] * n))
+        ks, vs = (stands_for(x, BF16).astype(np.float64) for x in (k, v))
+        s = np.einsum("hgd,phd->hgp", q[0].astype(np.float64).reshape(hk, h // hk, d), ks) * scale
+        margin = sign * (s[..., at, None] - np.delete(s, at, -1))
+        assert (margin > 1e6).all()  # e^-margin is nothing, whatever the rounding of the scores
+        want, bound = attend(q[0], ks, vs, np.array([at]) if sign > 0 else np.delete(np.arange(n), at), scale)
+        if sign > 0:
+            bound = 2.0 ** -20 * np.abs(want)
+        got = run_attention(kv, q, [n], table, scale=scale).cpu().numpy().astype(np.float64).reshape(h, d)
+        assert (np.abs(got - want) <= bound).all()
+        kv.free()
