@@ -83,6 +83,9 @@ struct PagedCfg {
     // Queries are scaled into [2^QLIFT, 2^(QLIFT + 1)): f16 parts as high as their range allows; bf16
     // parts have f32's range and stay so low that no finite key overflows a sum of 256 products.
     static constexpr int QLIFT = NS == 3 ? -10 : 13;
+    // bf16 weights are relative to 2^UP times the maximum when it was last raised: with kLazy they stay
+    // below 2^-16, and sums of 65536 values of any finite size below f32's largest number.
+    static constexpr float UP = NS == 3 ? 32.0f : 0.0f;
     static constexpr float CODE = TYPE == SSD_TYPE_Q8_0 ? 16777216.0f : 1.0f;  // code / fragment
     static constexpr int HALF = paged_half_bytes(TYPE, HD);  // bytes of a group's K, or V
     static constexpr int ROW = HD + 4;                       // floats of a head in a partial
@@ -775,7 +778,7 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                 for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) acc[b][i][j] = 0.0f;
-            float m = -INFINITY, l = 0.0f;  // of head g
+            float m = -INFINITY, l = 0.0f;  // of head g (m with UP)
             // V's scales are multiplied by 2^k (dk), the products with P by 2^-k 2^-kLift (unlift)
             float dref = 0.0f, unlift = kUnlift * C::CODE;
             uint32_t dk = 0;
@@ -876,7 +879,7 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                 // weights are 2^(x c1 - base): relative to the tile's largest, or to m
                 float base = NS == 3 ? (m == -INFINITY ? 0.0f : m) : (mx == -INFINITY ? 0.0f : mx - kLift);
                 const bool large = (__float_as_uint(mx) & 0x7FFFFFFFu) - kLargeFrom < kLargeTo - kLargeFrom;
-                bool update = mx > m + kLazy || large, again = false;
+                bool update = mx > m + (kLazy - C::UP) || large, again = false;
                 float dm = 0.0f;
                 if constexpr (C::QT) {
                     dm = T[0].v_scale_max();
@@ -897,7 +900,7 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                     }
                     if (__any_sync(0xffffffffu, update)) {
-                        const float mn = fmaxf(m, mx);
+                        const float mn = fmaxf(m, mx + C::UP);
                         const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
                         m = mn;
                         if constexpr (NS == 3) base = m == -INFINITY ? 0.0f : m;
