@@ -60,11 +60,20 @@ namespace ssd {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kMask8 = 0x807F807Fu;  // 8-bit codes as f16: q 2^-24 (paged.cuh)
-// f16 weights: relative to the tile's largest, which is 2^kLift; those below kSmall take another
-// pass, multiplied by kStep (so that each pass has 24 binades, 11 of f16's mantissa bits above its
-// smallest number at the lower end).
-constexpr float kLift = 13.0f, kUnlift = 1.0f / 8192.0f;
-constexpr float kSmall = 1.0f / 2048.0f, kSmallLog = -11.0f, kStep = 16777216.0f;
+// f16 weights: relative to the tile's largest (LIFT below); those under kSmall take another pass (so
+// that each pass has 24 binades, 13 of f16's mantissa bits above its smallest number at the lower end).
+constexpr float kSmall = 1.0f / 2048.0f, kSmallLog = -11.0f;
+// 8- and 4-bit caches: a weight meets its position's V scales as f16 numbers too, multiplied by 2^k,
+// so that each is below 2. Every product of the two other than zero is kProd or more in the pass that
+// takes it: of 13 bits at least, of 22 from 2^-3 on. That holds where no scale is under kScaleLow and
+// no weight under kProd / kScaleLow; else (one tile in twenty of normally distributed keys) each
+// weight is looked at with its own position's scales. Where one is too small (one in some hundreds),
+// a pass takes as many binades of weights as the tile's smallest scale leaves, and scales under
+// 2^-kBin have passes of their own.
+constexpr float kProd = 1.0f / 1024.0f, kScaleLow = 1.0f / 32.0f, kWeightLog = -5.0f;
+constexpr float kNormal = 1.0f / 16384.0f;  // f16's smallest number of 11 bits
+constexpr int kBin = 7;
+constexpr float kBinSmall = 0.125f, kBinStep = 256.0f;  // kProd 2^kBin, 2^(kBin + 1)
 // Products with q become scores within the subtraction of the tile's largest score, in one rounding;
 // the largest one has a rounding of its own, a sixteenth at 2^20 and without bound above. Where it is
 // larger (2^20 to infinity, as bits of its magnitude), the largest product is subtracted first.
@@ -87,6 +96,11 @@ struct PagedCfg {
     // 12 bits.
     static constexpr float LAZY = NS == 3 ? 2.0f : 16.0f;
     static constexpr float UP = NS == 3 ? 6.0f : 0.0f;
+    // f16 weights are relative to the tile's largest, which is 2^LIFT (DOWN: the inverse): times a scale
+    // below 2 and 2^(1/16), what a score may be off, it has to stay an f16 number.
+    static constexpr float LIFT = QT ? 14.875f : 13.0f;
+    static constexpr float DOWN = QT ? 3.3279655e-5f : 1.0f / 8192.0f;
+    static constexpr int PASS = (int)LIFT;  // a pass's weights begin at 2^PASS
     static constexpr float CODE = TYPE == SSD_TYPE_Q8_0 ? 16777216.0f : 1.0f;  // code / fragment
     static constexpr int HALF = paged_half_bytes(TYPE, HD);  // bytes of a group's K, or V
     static constexpr int ROW = HD + 4;                       // floats of a head in a partial
@@ -290,12 +304,12 @@ struct PagedGroup {
             }
         }
     }
-    __device__ __forceinline__ void read_v_scales() {
+    // (from: where in the slot they lie)
+    __device__ __forceinline__ void read_v_scales(int from) {
         if constexpr (C::QT) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const uint8_t* r = slot + C::HALF + paged_elem_bytes(TYPE, HD) +
-                                   ((lane & 3) + 4 * i) * C::NB * 4;
+                const uint8_t* r = slot + from + ((lane & 3) + 4 * i) * C::NB * 4;
                 if constexpr (C::NB % 4 == 0) {
 #pragma unroll
                     for (int j = 0; j < C::NB / 4; j++) {
@@ -352,13 +366,13 @@ struct PagedGroup {
             }
         }
     }
-    // Largest magnitude of the lane's V scales.
-    __device__ __forceinline__ float v_scale_max() const {
-        __half2 m = TYPE == SSD_TYPE_Q4_0 ? __habs2(bits_h2(vs[0])) : bits_h2(vs[0]);
+    // Smallest magnitudes other than zero of V's scales at positions 2t and 2t + 1 (8 more: p = 1), as f16
+    // bits (zero: there is none). Zero is the largest 16-bit integer when 2^15 - 1 is added.
+    __device__ __forceinline__ uint32_t v_scale_min(int p) const {
+        uint32_t m = 0x7FFF7FFFu;
 #pragma unroll
-        for (int i = 1; i < 2 * C::NB; i++)
-            m = __hmax2(m, TYPE == SSD_TYPE_Q4_0 ? __habs2(bits_h2(vs[i])) : bits_h2(vs[i]));
-        return fmaxf(__low2float(m), __high2float(m));
+        for (int b = 0; b < C::NB; b++) m = __vmins2(m, (vs[p * C::NB + b] & 0x7FFF7FFFu) + 0x7FFF7FFFu);
+        return (m & 0xFFFFu) - 0x7FFFu & 0xFFFFu | (m >> 16) - 0x7FFFu << 16;
     }
 };
 
@@ -780,9 +794,9 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
 #pragma unroll
                     for (int j = 0; j < 4; j++) acc[b][i][j] = 0.0f;
             float m = -INFINITY, l = 0.0f;  // of head g (m with UP)
-            // V's scales are multiplied by 2^k (dk), the products with P by 2^-k 2^-kLift (unlift)
-            float dref = 0.0f, unlift = kUnlift * C::CODE;
-            uint32_t dk = 0;
+            // V's scales are multiplied by 2^k (dk: twice, as f16), the products with P by 2^-k DOWN (unlift)
+            uint32_t dk = 0x78007800u, scale_low = 0x00100010u;  // k = 15; kScaleLow 2^-k
+            float unlift = C::QT ? C::CODE * C::DOWN / 32768.0f : C::DOWN;
             for (int i = 0; i < n; i++) {
                 ring_wait(full0 + slot * 8, phase, tries, a.status);
                 PagedGroup<TYPE, HD, PACK> T[TP];
@@ -791,6 +805,49 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                 for (int j = 0; j < TP; j++) {
                     T[j].slot = ring + (slot * TP + j) * G;
                     T[j].lane = lane;
+                }
+                const int p0 = (rw.tile0 + tile + i) * TILE;
+                const uint32_t miss = missing >> 2 * slot & 3u;
+                auto inside = [&](int j) {  // of the lane's positions of group j
+                    uint32_t ok = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int p = p0 + 16 * j + 2 * t + (k & 1) + 8 * (k >> 1);
+                        if (!(miss >> j & 1) && p >= rw.start && p < rw.end) ok |= 1u << k;
+                    }
+                    return ok;
+                };
+                const bool part = miss || p0 < rw.start || rw.end - p0 < TILE;
+                // The tile's V scales as 32-bit words (two positions of a block), in the order of pairs,
+                // then blocks: the lane's share of them, without those of positions outside the range.
+                constexpr int WORDS = NB * 8, SHARE = (TP * WORDS + 31) / 32;
+                auto word_of = [&](int i) {  // (some lanes: one twice)
+                    const int at = i * 32 + lane;
+                    return at < TP * WORDS ? at : lane;
+                };
+                auto word_at = [&](int at, int of) {  // of: C::HALF, or 0: in the place of K's scales
+                    const int j = at / WORDS;
+                    return reinterpret_cast<uint32_t*>(T[0].slot + j * G + of + paged_elem_bytes(TYPE, HD)) +
+                           (at - j * WORDS);
+                };
+                auto scales = [&](int i) -> uint32_t {
+                    const int at = word_of(i), j = at / WORDS, p = p0 + 16 * j + 2 * ((at - j * WORDS) / NB);
+                    uint32_t d = *word_at(at, C::HALF);
+                    if (part && ((miss >> j & 1) || p < rw.start || p >= rw.end)) d &= 0xFFFF0000u;
+                    if (part && ((miss >> j & 1) || p + 1 < rw.start || p + 1 >= rw.end)) d &= 0x0000FFFFu;
+                    return d;
+                };
+                bool odd = part;  // a scale, times 2^k, may be 2 or more or under kScaleLow
+                __half2 hi, lo;
+                if constexpr (C::QT) {
+#pragma unroll
+                    for (int i = 0; i < SHARE; i++) {
+                        uint32_t d = *word_at(word_of(i), C::HALF);
+                        if constexpr (TYPE == SSD_TYPE_Q4_0) d &= 0x7FFF7FFFu;
+                        hi = i ? __hmax2(hi, bits_h2(d)) : bits_h2(d);
+                        lo = i ? __hmin2(lo, bits_h2(d)) : bits_h2(d);
+                    }
+                    odd |= !__hblt2(hi, bits_h2(0x7C007C00u - dk)) || !__hbge2(lo, bits_h2(scale_low));
                 }
                 // Q K
                 {
@@ -850,21 +907,14 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                         }
                 }
 #pragma unroll
-                for (int j = 0; j < TP; j++) T[j].read_v_scales();
-                const int p0 = (rw.tile0 + tile + i) * TILE;
-                const uint32_t miss = missing >> 2 * slot & 3u;
-                if (miss || p0 < rw.start || rw.end - p0 < TILE) {
+                for (int j = 0; j < TP; j++) T[j].read_v_scales(C::HALF + paged_elem_bytes(TYPE, HD));
+                if (part) {
 #pragma unroll
                     for (int j = 0; j < TP; j++) {
-                        uint32_t ok = 0;
+                        const uint32_t ok = inside(j);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const int p = p0 + 16 * j + 2 * t + (k & 1) + 8 * (k >> 1);
-                            if (!(miss >> j & 1) && p >= rw.start && p < rw.end)
-                                ok |= 1u << k;
-                            else
-                                x[j][k] = -INFINITY;
-                        }
+                        for (int k = 0; k < 4; k++)
+                            if (!(ok >> k & 1)) x[j][k] = -INFINITY;
                         T[j].mask_v(ok);
                     }
                 }
@@ -878,23 +928,34 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                 }
                 mx *= c1;
                 // weights are 2^(x c1 - base): relative to the tile's largest, or to m
-                float base = NS == 3 ? (m == -INFINITY ? 0.0f : m) : (mx == -INFINITY ? 0.0f : mx - kLift);
+                float base = NS == 3 ? (m == -INFINITY ? 0.0f : m) : (mx == -INFINITY ? 0.0f : mx - C::LIFT);
                 const bool large = (__float_as_uint(mx) & 0x7FFFFFFFu) - kLargeFrom < kLargeTo - kLargeFrom;
                 bool update = mx > m + (C::LAZY - C::UP) || large, again = false;
-                float dm = 0.0f;
-                if constexpr (C::QT) {
-                    dm = T[0].v_scale_max();
-                    if constexpr (TP == 2) dm = fmaxf(dm, T[TP - 1].v_scale_max());
-                    update |= dm > 2.0f * dref;
-                }
                 if constexpr (NS == 2) {
                     float mn = INFINITY;
 #pragma unroll
                     for (int j = 0; j < TP; j++)
                         mn = fminf(mn, fminf(fminf(x[j][0], x[j][1]), fminf(x[j][2], x[j][3])));
-                    again = fmaf(mn, c1, -base) < kSmallLog;
+                    const float low = fmaf(mn, c1, -base);  // log2 of the lane's smallest weight
+                    again = low < (C::QT ? kWeightLog : kSmallLog);
                 }
-                if (__any_sync(0xffffffffu, update || again)) {
+                if (__any_sync(0xffffffffu, update || again || (C::QT && odd))) {
+                    if constexpr (C::QT) {
+                        if (__any_sync(0xffffffffu, odd)) {  // 2^k for this tile: its largest scale to [1, 2)
+                            uint32_t top = 0;
+#pragma unroll
+                            for (int i = 0; i < SHARE; i++) {
+                                const uint32_t d = scales(i) & 0x7FFF7FFFu;
+                                top = max(top, max(d & 0xFFFFu, d >> 16));
+                            }
+                            const int e = max(30 - (int)(__reduce_max_sync(0xffffffffu, top) >> 10), 0);  // k + 15
+                            dk = e ? (uint32_t)e * 0x04000400u : 0x02000200u;
+                            const float down = __uint_as_float((uint32_t)(142 - e) << 23);  // 2^-k
+                            unlift = down * (C::CODE * C::DOWN);
+                            scale_low = __half_as_ushort(__float2half_rn(kScaleLow * down)) * 0x10001u;
+                            again |= part || !__hbge2(lo, bits_h2(scale_low));
+                        }
+                    }
                     again = __any_sync(0xffffffffu, again);
                     if constexpr (NS == 3) {
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -914,17 +975,6 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                             for (int i = 0; i < 2; i++)
 #pragma unroll
                                 for (int j = 0; j < 4; j++) acc[b][i][j] *= j & 1 ? f1 : f0;
-                        if constexpr (C::QT) {
-                            dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 1));
-                            dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 2));
-                            if (dm > 2.0f * dref) {  // 2^k dm in [1, 2), as far as f16 has 2^k
-                                dref = dm;
-                                const int k = min(15, max(-14, 127 - (int)(__float_as_uint(dm) >> 23)));
-                                dk = (uint32_t)(k + 15) << 10;
-                                dk |= dk << 16;
-                                unlift = __uint_as_float((uint32_t)(127 - 13 - k) << 23) * C::CODE;
-                            }
-                        }
                         if (__any_sync(0xffffffffu, large)) {
                             float top = -INFINITY;
 #pragma unroll
@@ -933,7 +983,7 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                             if (top > -INFINITY) {
-                                base = NS == 3 ? m - mx : -kLift;
+                                base = NS == 3 ? m - mx : -C::LIFT;
 #pragma unroll
                                 for (int j = 0; j < TP; j++)
 #pragma unroll
@@ -952,32 +1002,15 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                 if constexpr (TP == 2) sum += (w[TP - 1][0] + w[TP - 1][1]) + (w[TP - 1][2] + w[TP - 1][3]);
                 if constexpr (NS == 2) {
                     const float beta = m == -INFINITY ? 0.0f : ex2(mx - m);
-                    l = fmaf(sum, beta * kUnlift, l);
+                    l = fmaf(sum, beta * C::DOWN, l);
                     fa = __shfl_sync(0xffffffffu, beta, 8 * t) * unlift;
                     fb = __shfl_sync(0xffffffffu, beta, 8 * t + 4) * unlift;
                 } else {
                     l += sum;
                 }
-                // P V, for f16 weights in as many passes as their range needs (one, as a rule)
-                do {
-                    float u[TP][4];
-#pragma unroll
-                    for (int j = 0; j < TP; j++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) u[j][k] = w[j][k];
-                    if (again) {
-                        again = false;
-#pragma unroll
-                        for (int j = 0; j < TP; j++)
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                const bool small = w[j][k] < kSmall;
-                                again |= small && w[j][k] > 0.0f;
-                                u[j][k] = small ? 0.0f : w[j][k];
-                                w[j][k] = small ? w[j][k] * kStep : 0.0f;
-                            }
-                        again = __any_sync(0xffffffffu, again);
-                    }
+                // P V; for f16 weights in as many passes as their range needs (one, as a rule; the others
+                // in a copy of the code, which leaves the rule's without a loop)
+                auto products = [&](const float (&u)[TP][4]) {
                     uint32_t pu[TP][2][NS];
 #pragma unroll
                     for (int j = 0; j < TP; j++)
@@ -1023,11 +1056,83 @@ __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
                                                        : acc[b][h][k] + c[k];
                         }
                     }
-                    if constexpr (NS == 2) {
-                        fa *= 1.0f / kStep;
-                        fb *= 1.0f / kStep;
+                };
+                const float up = __uint_as_float(((dk >> 26) + 112) << 23);  // 2^k
+                if (NS == 2 && again) {
+                    again = false;
+#pragma unroll
+                    for (int j = 0; j < TP; j++)
+#pragma unroll
+                        for (int p = 0; p < 2; p++) {
+                            uint32_t least = 0;
+                            if constexpr (C::QT) least = T[j].v_scale_min(p);
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                const float d = f16_bits_to_f32((uint16_t)(least >> 16 * k)) * up, y = w[j][2 * p + k];
+                                again |= y > 0.0f && (C::QT ? d > 0.0f && (y * d < kProd || d < kNormal) : y < kSmall);
+                            }
+                        }
+                    again = __any_sync(0xffffffffu, again);
+                }
+                if (NS == 3 || !again) {
+                    products(w);
+                } else {
+                    float small = kSmall;  // a pass takes weights down to this
+                    if constexpr (C::QT) {
+                        uint32_t least = 0x7800u;  // f16 bits of the smallest scale other than zero, less one
+#pragma unroll
+                        for (int i = 0; i < SHARE; i++) {
+                            const uint32_t d = scales(i) & 0x7FFF7FFFu;
+                            least = min(least, min((d & 0xFFFFu) - 1u, (d >> 16) - 1u));
+                        }
+                        least = __reduce_min_sync(0xffffffffu, least);
+                        const int e = (int)(__float_as_uint(f16_bits_to_f32((uint16_t)least) * up) >> 23);
+                        small = e < 127 - kBin ? kBinSmall : kProd * __uint_as_float((uint32_t)(254 - e) << 23);
                     }
-                } while (again);
+                    float by = 1.0f;  // the pass's factor on the scales
+                    do {
+                        float u[TP][4], next;  // fa, fb to the next pass's
+                        bool rest = false;     // smaller scales have to meet the same weights
+                        if constexpr (C::QT) {
+                            if (small == kBinSmall) {  // this pass's scales, in the place of K's
+                                constexpr float from = 1.0f / (1 << kBin);
+                                const float to = by == 1.0f ? NAN : from * kBinStep;  // (the first: all above)
+                                __syncwarp();
+#pragma unroll
+                                for (int i = 0; i < SHARE; i++) {
+                                    const float2 d = __half22float2(bits_h2(scales(i)));
+                                    const float y = fabsf(d.x) * (up * by), z = fabsf(d.y) * (up * by);
+                                    rest |= (y > 0.0f && y < from) || (z > 0.0f && z < from);
+                                    *word_at(word_of(i), 0) =
+                                        h2bits(__floats2half2_rn(y < from || y >= to ? 0.0f : d.x * by,
+                                                                 z < from || z >= to ? 0.0f : d.y * by));
+                                }
+                                rest = __any_sync(0xffffffffu, rest);
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // as mask_v
+                                __syncwarp();
+#pragma unroll
+                                for (int j = 0; j < TP; j++) T[j].read_v_scales(paged_elem_bytes(TYPE, HD));
+                            }
+                        }
+                        const float step = __uint_as_float(((uint32_t)(254 + C::PASS) << 23) - __float_as_uint(small));
+                        again = false;
+#pragma unroll
+                        for (int j = 0; j < TP; j++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const bool later = w[j][k] < small;
+                                again |= later && w[j][k] > 0.0f;
+                                u[j][k] = later ? 0.0f : w[j][k];
+                                if (!rest) w[j][k] = later ? w[j][k] * step : 0.0f;
+                            }
+                        again = rest || __any_sync(0xffffffffu, again);
+                        next = rest ? 1.0f / kBinStep : by * (small / (1 << C::PASS));
+                        by = rest ? by * kBinStep : 1.0f;
+                        products(u);
+                        fa *= next;
+                        fb *= next;
+                    } while (again);
+                }
                 __syncwarp();  // the slot is read
                 ask(slot);
                 if (++slot == S) {

@@ -942,3 +942,95 @@ def test_small_weights_beside_a_bf16_cache(ctx, nats, d, group):
     held = [tuple(stands_for(x, BF16).astype(np.float64) for x in (k, v))]
     check_attention(run_attention(kv, q, [n], table), q, held, [n])
     kv.free()
+
+
+def hold(ctx, rng, k, v, page, wtype):
+    """A cache that holds k and v of one sequence; its table and the held values."""
+    n, hk, d = k.shape
+    pages = n // page + 2
+    kv = ssdllm.PagedKvCache(ctx, pages, page, hk, d, wtype)
+    table = make_table(rng, [n], page, pages)
+    k, v = k.astype(np.float32), v.astype(np.float32)
+    kv.append(torch.from_numpy(k).to(DEV), torch.from_numpy(v).to(DEV), i32(np.arange(n)), i32(table),
+              seq=i32([0] * n))
+    return kv, table, [tuple(stands_for(x, wtype).astype(np.float64) for x in (k, v))]
+
+
+@pytest.mark.parametrize("wtype", TYPES)
+@pytest.mark.parametrize("nats", [8, 14, 17, 25, 40, 75])
+@pytest.mark.parametrize("d,group", [(64, 3), (128, 8), (256, 5)])
+def test_a_strong_position_with_zero_values(ctx, wtype, nats, d, group):
+    """One position's score is far above the others' and its V is zero: what counts are weights far
+    below the largest, alone and beside values 2^8 to 2^20 times as large of positions with no weight
+    to speak of, of other blocks of dims, or of the same tile's positions."""
+    rng = np.random.default_rng(27)
+    n, hk = 200, 2
+    q = (rng.random((1, group * hk, d)) + 0.5).astype(np.float32)
+    k1 = 0.002 * rng.standard_normal((n, hk, d))
+    k1[70] = nats / (d * d ** -0.5)
+    v1 = rng.standard_normal((n, hk, d))
+    v1[70] = 0.0
+    for shape in ("equal", "before", "blocks", "ragged"):
+        for size in (2.0 ** 8, 2.0 ** 12, 2.0 ** 20):
+            k, v = k1.copy(), v1.copy()
+            if size > 2.0 ** 15:
+                v *= 2.0 ** -8  # f16 ends at 2^16
+            if shape == "before":     # tiles before it and its own
+                k[[3, 66]] = -60 / (d * d ** -0.5)
+                v[[3, 66]] *= size
+            elif shape == "blocks":   # dims 32 to 63
+                v[:, :, 32:64] *= size
+            elif shape == "ragged":   # every other position
+                k[::2] += -20 / (d * d ** -0.5)
+                v[::2] *= size
+                v[70] = 0.0
+            kv, table, held = hold(ctx, rng, k, v, 32, wtype)
+            check_attention(run_attention(kv, q, [n], table), q, held, [n])
+            check_attention(run_attention(kv, q, [75], table, window=30), q, held, [75], window=30)
+            kv.free()
+            if shape == "equal":
+                break
+
+
+@pytest.mark.parametrize("wtype", [Q8, Q4])
+@pytest.mark.parametrize("top", [2.0 ** 18, 1.0, 2.0 ** -10])
+@pytest.mark.parametrize("nats", [0, 5, 30])
+def test_value_scales_of_every_size(ctx, wtype, top, nats):
+    """V whose blocks' scales go through all of f16's range and are zero, under equal and very different
+    weights: every block's output is in proportion to what is in that block."""
+    rng = np.random.default_rng(28)
+    n, hk, h, d = 333, 1, 4, 256
+    q = (rng.random((1, h, d)) + 0.5).astype(np.float32)
+    k = 0.002 * rng.standard_normal((n, hk, d)) - np.linspace(0, nats, n)[:, None, None] / (d * d ** -0.5)
+    top = min(top, 2.0 ** 15) if wtype == Q4 else top  # a scale is the largest value's eighth, and an f16 number
+    v = rng.standard_normal((n, hk, d)) * top * np.repeat(2.0 ** -np.arange(0, 32, 4), 32)
+    v[100:200] = 0.0
+    v[:, :, 64:96] *= 2.0 ** -rng.integers(0, 12, (n, 1, 1))
+    kv, table, held = hold(ctx, rng, k, v, 16, wtype)
+    check_attention(run_attention(kv, q, [n], table), q, held, [n])
+    kv.free()
+
+
+@pytest.mark.parametrize("wtype", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_nan_and_infinite_values_beside_small_weights(ctx, wtype, bad):
+    """A V that is not a number makes its block's outputs so, not others', when weights need passes of
+    their own; outside the range it does not matter."""
+    rng = np.random.default_rng(29)
+    n, d = 90, 64
+    q = (rng.random((1, 4, d)) + 0.5).astype(np.float32)
+    k = 0.002 * rng.standard_normal((n, 1, d))
+    k[40] = 30 / 8
+    v = rng.standard_normal((n, 1, d)) * np.repeat([1.0, 2.0 ** 12], 32)
+    v[60:, :, :32] = 3e38 if wtype != F16 and wtype != BF16 and bad > 0 else bad  # 8- and 4-bit codes of NaN are numbers
+    if wtype in (Q8, Q4) and bad != bad:
+        v[60:, :, :32] = np.inf
+    with np.errstate(all="ignore"):
+        kv, table, held = hold(ctx, rng, k, v, 16, wtype)
+        out = run_attention(kv, q, [60], table).view(4, d)
+        check_attention(out[None], q, [(held[0][0][:60], held[0][1][:60])], [60])
+        out = run_attention(kv, q, [n], table).cpu().numpy().astype(np.float64).reshape(4, d)
+        assert not np.isfinite(out[:, :32]).any()
+        ref, bound = attend(q[0], held[0][0], np.concatenate([np.zeros((n, 1, 32)), held[0][1][:, :, 32:]], -1))
+        assert (np.abs(out - ref)[:, 32:] <= bound[:, 32:]).all()
+    kv.free()
