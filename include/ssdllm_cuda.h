@@ -308,9 +308,9 @@ int ssd_attention_prefill(ssd_ctx* ctx, const ssd_kv_cache* kv, const float* q_d
  * the calls for contiguous caches refuse it (SSD_ERR_STATE). Pages start as zeros.
  *
  * The calls below take rows: row r belongs to sequence seq_dev[r] (seq_dev NULL: to sequence r)
- * and its strides are in elements. n_rows 0 is a no-op. No call allocates; all are stream-ordered
- * and may be captured into a graph, after a first call on a cache of the same type and head_dim
- * (which loads the kernels). */
+ * and its strides are in elements. n_rows 0 is a no-op. No call but the creation allocates; all are
+ * stream-ordered, and those on a cache may be captured into a graph from the first one on (the
+ * creation loads the kernels of its type and head_dim). */
 int ssd_kv_create_paged(ssd_ctx* ctx, int n_pages, int page_size, int n_head_kv, int head_dim,
                         int ggml_type, ssd_kv_cache** out);
 /* Rotation table for ssd_paged_append: table_dev[n_positions][rope_dim / 2] pairs (cos, sin) of

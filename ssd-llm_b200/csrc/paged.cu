@@ -645,6 +645,18 @@ struct ReadLaunch {
     }
 };
 
+struct CacheLoad {
+    template <int TYPE, int HD>
+    int run() const {
+        cudaFuncAttributes at;
+        SSD_CK(cudaFuncGetAttributes(&at, k_paged_append<TYPE, HD, true>));
+        SSD_CK(cudaFuncGetAttributes(&at, k_paged_append<TYPE, HD, false>));
+        SSD_CK(cudaFuncGetAttributes(&at, k_paged_read<TYPE, HD, true>));
+        SSD_CK(cudaFuncGetAttributes(&at, k_paged_read<TYPE, HD, false>));
+        return load_paged_attention(TYPE, HD);
+    }
+};
+
 }  // namespace ssd
 
 using namespace ssd;
@@ -664,6 +676,7 @@ extern "C" int ssd_kv_create_paged(ssd_ctx* ctx, int n_pages, int page_size, int
     const uint64_t total = (uint64_t)n_pages * n_head_kv * head;
     SSD_REQ((double)n_pages * n_head_kv * (double)head < 1e15, SSD_ERR_NOMEM,
             "paged KV cache of %d pages is too large", n_pages);
+    SSD_TRY(paged_dispatch(ggml_type, head_dim, CacheLoad{}));
     void* p = nullptr;
     if (cudaMalloc(&p, total) != cudaSuccess) {
         cudaGetLastError();

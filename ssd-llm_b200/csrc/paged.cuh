@@ -232,6 +232,9 @@ struct PagedAttnArgs {
     bool q_vec, out_vec;  // rows start on 16-byte boundaries
 };
 size_t paged_attn_workspace(const ssd_ctx* ctx, int head_dim);
+// Loads what the calls on a cache of this type and head size may launch, on the current device: with
+// lazy loading the first launch of a kernel would do it, which a stream capture may not allow.
+int load_paged_attention(int type, int head_dim);
 int launch_paged_attention(ssd_ctx* ctx, int type, int head_dim, const PagedAttnArgs& a,
                            cudaStream_t s, bool pdl);
 

@@ -52,8 +52,6 @@
 #include <float.h>
 #include <limits.h>
 
-#include <atomic>
-
 #include "paged.cuh"
 
 namespace ssd {
@@ -1327,18 +1325,28 @@ struct AttnLaunch {
     template <int TYPE, int HD, bool PACK>
     int go() const {
         using C = PagedCfg<TYPE, HD, PACK>;
-        static std::atomic<uint64_t> ready{0};  // devices (bits) whose limit is raised
-        const uint64_t bit = 1ull << (ctx->device & 63);
-        if (ctx->device > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
-            SSD_CK(cudaFuncSetAttribute(k_paged_attn<TYPE, HD, PACK>,
-                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-            ready.fetch_or(bit, std::memory_order_relaxed);
-        }
         const int grid = ctx->num_sms;
         SSD_CK(launch_pdl(k_paged_attn<TYPE, HD, PACK>, dim3(grid), dim3(C::THREADS), C::SMEM, s, pdl, a));
         return SSD_OK;
     }
 };
+
+struct AttnLoad {
+    template <int TYPE, int HD>
+    int run() const {
+        SSD_TRY((go<TYPE, HD, true>()));
+        return go<TYPE, HD, false>();
+    }
+    template <int TYPE, int HD, bool PACK>
+    static int go() {
+        cudaFuncAttributes at;
+        SSD_CK(cudaFuncGetAttributes(&at, k_paged_attn<TYPE, HD, PACK>));
+        SSD_CK(cudaFuncSetAttribute(k_paged_attn<TYPE, HD, PACK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    PagedCfg<TYPE, HD, PACK>::SMEM));
+        return SSD_OK;
+    }
+};
+int load_paged_attention(int type, int head_dim) { return paged_dispatch(type, head_dim, AttnLoad{}); }
 
 size_t paged_attn_workspace(const ssd_ctx* ctx, int head_dim) {
     const int ctas = ctx->num_sms;

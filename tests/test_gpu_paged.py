@@ -10,6 +10,10 @@ Tolerances, from the arithmetic (eps = 2^-24, the error of one f32 rounding):
   S = scale * sum |q||k| (32 roundings); weights move by twice the largest score error, and the
   weighted sum and its division add 2^-20: |out - exact| <= (2 * 2^-19 max S + 2^-20) sum w |v|.
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -1034,3 +1038,50 @@ def test_nan_and_infinite_values_beside_small_weights(ctx, wtype, bad):
         ref, bound = attend(q[0], held[0][0], np.concatenate([np.zeros((n, 1, 32)), held[0][1][:, :, 32:]], -1))
         assert (np.abs(out - ref)[:, 32:] <= bound[:, 32:]).all()
     kv.free()
+
+
+FIRST_CALLS = '''
+import sys
+import torch
+import ssdllm
+wtype, d = int(sys.argv[1]), int(sys.argv[2])
+ctx = ssdllm.Context(0)
+dev = torch.device("cuda", 0)
+kv = ssdllm.PagedKvCache(ctx, 4, 16, 2, d, wtype)
+i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+table, pos, length, seq = i32([[0, 1, 2, 3]]), i32([5]), i32([6]), i32([0])
+work = kv.attention_workspace()
+bufs = []
+for off in (0, 1):  # rows on 16-byte boundaries, and not
+    for group in (4, 8):
+        w = [torch.randn(1, n + 1, device=dev)[:, off:off + n] for n in (2 * d, 2 * d, 2 * group * d, 2 * group * d)]
+        bufs.append(w + [torch.empty(1, 2 * d + 1, device=dev)[:, off:off + 2 * d] for _ in range(2)] +
+                    [torch.full((1, 2 * group * d + 1), float("nan"), device=dev)[:, off:off + 2 * group * d]])
+torch.cuda.synchronize()
+def calls():
+    for k, v, q, qo, ko, vo, out in bufs:
+        kv.append(k, v, pos, table, seq=seq, q=q, q_out=qo)
+        kv.read(pos, table, ko, vo, seq=seq)
+        kv.attention(qo, length, table, out, work, seq=seq)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    calls()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for b in bufs for t in b[3:]]
+assert all(torch.isfinite(t).all() for t in got)
+calls()
+torch.cuda.synchronize()
+assert all(torch.equal(a, t) for a, t in zip(got, [t for b in bufs for t in b[3:]]))
+assert ctx.device_status() == 0
+'''
+
+
+@pytest.mark.parametrize("wtype,d", [(F16, 64), (BF16, 128), (Q8, 128), (Q4, 96)])
+def test_the_first_calls_on_a_cache_may_be_captured(ctx, wtype, d):
+    """In a process of its own: whatever the group of queries and the rows' alignment are, no call on
+    the cache has to come before a capture."""
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ssd-llm_b200")
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS, str(wtype), str(d)], capture_output=True, text=True,
+                       timeout=120, env={**os.environ, "PYTHONPATH": root, "CUDA_MODULE_LOADING": "LAZY"})
+    assert r.returncode == 0, r.stderr[-2000:]
