@@ -482,23 +482,23 @@ def rope_table(ctx, rope_dim: int, theta: float, n_positions: int, table):
     if table.numel() != n_positions * rope_dim:
         raise SsdError(1, f"table of {table.numel()} values, {n_positions * rope_dim} needed")
     import torch
-    check(lib().ssd_rope_table(ctx.h, rope_dim, theta, n_positions, _flat(table, torch.float32),
-                               _stream()))
+    check(lib().ssd_rope_table(ctx.h, rope_dim, theta, n_positions,
+                               _flat(table, torch.float32, ctx.device), _stream_of(ctx.device)))
 
 
-def _flat(t, dtype):
-    """Address of a contiguous CUDA tensor of this type (None: null)."""
+def _flat(t, dtype, device):
+    """Address of a contiguous tensor of this type on this GPU (None: null)."""
     if t is None:
         return None
-    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
-        raise SsdError(1, f"a contiguous {dtype} CUDA tensor is wanted, got {t.dtype} "
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        raise SsdError(1, f"a contiguous {dtype} tensor on cuda:{device} is wanted, got {t.dtype} "
                           f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
     return t.data_ptr()
 
 
-def _rows(t, dtype, width=None):
-    """(address, row stride, rows, width) of a CUDA tensor [rows][width] or
-    [rows][heads][head_dim] whose rows are contiguous."""
+def _rows(t, dtype, device, width=None):
+    """(address, row stride, rows, width) of a tensor on this GPU, [rows][width] or
+    [rows][heads][head_dim], whose rows are contiguous."""
     shape, stride = t.shape, t.stride()
     if len(shape) == 2:
         n, w = shape
@@ -508,9 +508,11 @@ def _rows(t, dtype, width=None):
         w, ok = heads * d, stride[2] == 1 and (heads == 1 or stride[1] == d)
     else:
         n, w, ok = 0, 0, False
-    if not ok or t.dtype is not dtype or not t.is_cuda or (width is not None and w != width):
-        raise SsdError(1, f"rows of {'' if width is None else width} {dtype} values on a GPU are "
-                          f"wanted, got {t.dtype} {tuple(shape)} strides {stride} on {t.device}")
+    if not ok or t.dtype is not dtype or t.get_device() != device or \
+            (width is not None and w != width):
+        raise SsdError(1, f"rows of {'' if width is None else width} {dtype} values on "
+                          f"cuda:{device} are wanted, got {t.dtype} {tuple(shape)} strides {stride} "
+                          f"on {t.device}")
     # the stride of a single row says nothing
     return t.data_ptr(), stride[0] if n > 1 else max(w, stride[0]), n, w
 
@@ -535,13 +537,13 @@ class PagedKvCache:
         self.n_head_kv, self.head_dim = n_head_kv, head_dim
 
     def _table(self, table, seq, index, n_rows):
-        shape, i32 = table.shape, self.torch.int32
+        shape, i32, dev = table.shape, self.torch.int32, self.ctx.device
         if len(shape) != 2:
             raise SsdError(1, f"a page table [sequences][pages] is wanted, got {tuple(shape)}")
         if index.numel() != n_rows or (seq is not None and seq.numel() != n_rows):
             raise SsdError(3, f"{index.numel()} positions or lengths, "
                               f"{'no' if seq is None else seq.numel()} sequences for {n_rows} rows")
-        return _flat(index, i32), _flat(seq, i32), _flat(table, i32), shape[0], shape[1]
+        return _flat(index, i32, dev), _flat(seq, i32, dev), _flat(table, i32, dev), shape[0], shape[1]
 
     def append(self, k, v, pos, table, seq=None, q=None, q_out=None, q_norm=None, k_norm=None,
                eps: float = 1e-5, rope=None, rope_halves: bool = False):
@@ -549,9 +551,9 @@ class PagedKvCache:
         rotation of the keys as given). With q (and q_out), [rows][n_head * head_dim], the
         queries' norm and rotation are done in the same pass. rope: [positions][rope_dim / 2][2]
         (cos, sin) from rope_table."""
-        w, f32 = self.n_head_kv * self.head_dim, self.torch.float32
-        kp, ks, n, _ = _rows(k, f32, w)
-        vp, vs, nv, _ = _rows(v, f32, w)
+        w, f32, dev = self.n_head_kv * self.head_dim, self.torch.float32, self.ctx.device
+        kp, ks, n, _ = _rows(k, f32, dev, w)
+        vp, vs, nv, _ = _rows(v, f32, dev, w)
         qp = op = None
         qs = os_ = heads = 0
         if nv != n:
@@ -559,9 +561,9 @@ class PagedKvCache:
         if (q is None) != (q_out is None):
             raise SsdError(1, "q and q_out go together")
         if q is not None:
-            qp, qs, nq, qw = _rows(q, f32)
+            qp, qs, nq, qw = _rows(q, f32, dev)
             heads = qw // self.head_dim
-            op, os_, no, _ = _rows(q_out, f32, heads * self.head_dim)
+            op, os_, no, _ = _rows(q_out, f32, dev, heads * self.head_dim)
             if nq != n or no != n or qw != heads * self.head_dim:
                 raise SsdError(3, f"q and q_out need {n} rows each of whole heads of {self.head_dim}")
         if (q_norm is not None and q_norm.numel() != self.head_dim) or \
@@ -575,22 +577,22 @@ class PagedKvCache:
             rp, rd = shape[0], 2 * shape[1]
         index, sq, tb, n_seq, pages = self._table(table, seq, pos, n)
         check(lib().ssd_paged_append(self.ctx.h, self.h, qp, qs, heads, kp, ks, vp, vs, n,
-                                     _flat(q_norm, f32), _flat(k_norm, f32), eps,
-                                     _flat(rope, f32), rd, rp, int(rope_halves), index, sq,
-                                     tb, n_seq, pages, op, os_, _stream_of(self.ctx.device)))
+                                     _flat(q_norm, f32, dev), _flat(k_norm, f32, dev), eps,
+                                     _flat(rope, f32, dev), rd, rp, int(rope_halves), index, sq,
+                                     tb, n_seq, pages, op, os_, _stream_of(dev)))
 
     def read(self, pos, table, k_out, v_out, seq=None):
         """The values at rows (seq, pos) into k_out, v_out [rows][n_head_kv * head_dim], float32,
         float16 or bfloat16."""
-        w, t, dt = self.n_head_kv * self.head_dim, self.torch, k_out.dtype
+        w, t, dt, dev = self.n_head_kv * self.head_dim, self.torch, k_out.dtype, self.ctx.device
         kind = F32 if dt is t.float32 else F16 if dt is t.float16 else BF16
-        kp, ks, n, _ = _rows(k_out, dt if kind != BF16 else t.bfloat16, w)
-        vp, vs, nv, _ = _rows(v_out, dt, w)
+        kp, ks, n, _ = _rows(k_out, dt if kind != BF16 else t.bfloat16, dev, w)
+        vp, vs, nv, _ = _rows(v_out, dt, dev, w)
         if nv != n:
             raise SsdError(3, f"k_out has {n} rows, v_out {nv}")
         index, sq, tb, n_seq, pages = self._table(table, seq, pos, n)
         check(lib().ssd_paged_read(self.ctx.h, self.h, n, index, sq, tb, n_seq, pages, kind, kp, ks,
-                                   vp, vs, _stream_of(self.ctx.device)))
+                                   vp, vs, _stream_of(dev)))
 
     def attention_workspace(self):
         """A workspace for attention(): one per stream that calls it."""
@@ -603,17 +605,17 @@ class PagedKvCache:
                   window: int = 0):
         """Attention of each row of q [rows][n_head * head_dim] over the first `length[row]`
         positions of its sequence (the last `window` of them if window > 0) into out."""
-        f32 = self.torch.float32
-        qp, qs, n, width = _rows(q, f32)
-        op, os_, no, _ = _rows(out, f32, width)
+        f32, dev = self.torch.float32, self.ctx.device
+        qp, qs, n, width = _rows(q, f32, dev)
+        op, os_, no, _ = _rows(out, f32, dev, width)
         if no != n or width % self.head_dim:
             raise SsdError(3, f"q {tuple(q.shape)} and out {tuple(out.shape)} do not fit heads of "
                               f"{self.head_dim}")
         index, sq, tb, n_seq, pages = self._table(table, seq, length, n)
         check(lib().ssd_paged_attention(self.ctx.h, self.h, qp, qs, width // self.head_dim, n,
                                         index, sq, tb, n_seq, pages, scale, window, op, os_,
-                                        _flat(workspace, self.torch.uint8), workspace.numel(),
-                                        _stream_of(self.ctx.device)))
+                                        _flat(workspace, self.torch.uint8, dev),
+                                        workspace.numel(), _stream_of(dev)))
 
     def free(self):
         if self.h:
