@@ -119,6 +119,11 @@ class Batch:
     def generate(self, requests):
         """requests: {id: (prompt tokens, new tokens)}; returns {id: generated tokens}."""
         waiting, done, m = list(requests.items()), {}, self.model
+        most = min(m.max_positions, m.n_pages * m.page_size)
+        for rid, (prompt, new) in waiting:  # none that no step would ever take up or end
+            if not prompt or new < 1 or len(prompt) + new > most:
+                raise ValueError(f"request {rid}: {len(prompt)} prompt and {new} new tokens, 1 or more of each "
+                                 f"and {most} together are possible")
         while waiting or any(self.run):
             for slot in range(self.slots):  # admit
                 if self.run[slot] is None and waiting:
