@@ -354,7 +354,8 @@ int ssd_paged_attention_workspace(ssd_ctx* ctx, const ssd_kv_cache* kv, size_t* 
  * sequence (a prompt's rows with len = position + 1). len_dev[r] <= 0 or a window without pages
  * gives zeros; lengths beyond the table are cut to it; positions whose page is missing are left
  * out. The work is split evenly over the GPU whatever the lengths are; SSD_ERR_SHAPE if
- * n_rows * (positions of a table row, or window) / 16 * KV heads reaches 2^31.
+ * n_rows * (P / 16 + 4) * n_head_kv * ceil(n_head / n_head_kv / 8) reaches 2^31, P the positions of
+ * a table row or, if that is less, the window (0: none), divided without remainder.
  * workspace_dev: ssd_paged_attention_workspace bytes, 16-byte aligned, filled with zeros once
  * before its first use; each call leaves it ready for the next. Calls that may overlap on the GPU
  * (two streams) need one each. */

@@ -1085,3 +1085,22 @@ def test_the_first_calls_on_a_cache_may_be_captured(ctx, wtype, d):
     r = subprocess.run([sys.executable, "-c", FIRST_CALLS, str(wtype), str(d)], capture_output=True, text=True,
                        timeout=120, env={**os.environ, "PYTHONPATH": root, "CUDA_MODULE_LOADING": "LAZY"})
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_the_largest_call_is_what_the_header_says(ctx):
+    """n_rows (P / 16 + 4) n_head_kv ceil(group / 8) below 2^31: one row more is refused."""
+    hk, group, pages = 2, 25, 1 << 22
+    kv = ssdllm.PagedKvCache(ctx, 2, 16, hk, 64, Q8)
+    table = torch.zeros(1, pages, dtype=torch.int32, device=DEV)
+    work = kv.attention_workspace()
+    for window in (0, 1 << 25):
+        most = (2 ** 31 - 1) // (((window or pages * 16) // 16 + 4) * hk * 4)
+        for n in (most, most + 1):
+            q = torch.zeros(n, hk * group * 64, device=DEV)
+            out, none = torch.full_like(q, float("nan")), i32([0] * n)
+            if n > most:
+                assert status(kv.attention, q, none, table, out, work, seq=none, window=window) == 3
+            else:
+                kv.attention(q, none, table, out, work, seq=none, window=window)
+                assert (out == 0).all()
+    kv.free()
