@@ -353,7 +353,8 @@ int ssd_paged_attention_workspace(ssd_ctx* ctx, const ssd_kv_cache* kv, size_t* 
  * n_head_kv), scores scaled by `scale` (0: 1 / sqrt(head_dim)). Several rows may name one
  * sequence (a prompt's rows with len = position + 1). len_dev[r] <= 0 or a window without pages
  * gives zeros; lengths beyond the table are cut to it; positions whose page is missing are left
- * out. The work is split evenly over the GPU whatever the lengths are; SSD_ERR_SHAPE if
+ * out. out_dev must not overlap q_dev. The work is split evenly over the GPU whatever the lengths
+ * are, every row on its own: rows of one sequence read its cache again each. SSD_ERR_SHAPE if
  * n_rows * (P / 16 + 4) * n_head_kv * ceil(n_head / n_head_kv / 8) reaches 2^31, P the positions of
  * a table row or, if that is less, the window (0: none), divided without remainder.
  * workspace_dev: ssd_paged_attention_workspace bytes, 16-byte aligned, filled with zeros once

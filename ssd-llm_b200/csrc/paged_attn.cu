@@ -12,12 +12,13 @@
 // tensor cores. tcgen05 would have 128 rows for 8 queries, and its accumulators would have to come
 // back from TMEM for the softmax of every few positions; register accumulators fit this shape.
 //
-// Shape of the work: a tile is 32 positions (two of the cache's groups; one where that
-// would leave too few warps) for one unit = (row, 8 query heads of one KV head). Each warp streams its tiles through a ring of its own in shared
-// memory, one bulk copy a tile (two for pages of 16 positions), into slots that the warp itself
-// frees: there is no barrier between warps and the copies run ahead across units. (Loading
-// fragments straight into registers, a tile ahead, kept too few bytes in flight; one more warp that
-// asks for everybody's copies could not keep up.)
+// Shape of the work: a tile is 32 positions (two of the cache's groups; one where that would leave
+// too few warps: 16-bit caches at heads of 128, all at wider ones) for one unit = (row, 8 query heads
+// of one KV head). Each warp streams its tiles through a ring of its own in shared memory, one bulk
+// copy a tile (two for pages of 16 positions), into slots that the warp itself frees: there is no
+// barrier between warps and the copies run ahead across units. (Loading fragments straight into
+// registers, a tile ahead, kept too few bytes in flight; one more warp that asks for everybody's
+// copies could not keep up.)
 //   S^T = K Q^T : A = K (16 positions x 16 dims), B = q (8 heads)
 //   O^T = V^T P^T : A = V^T (16 dims x 16 positions), B = P (8 heads), S^T transposed in between
 //   by 8x8 matrix moves.
@@ -27,28 +28,34 @@
 // positions, 32 / 8 heads, Q8_0: 80 -> 76 us; 32 rows over 4096, Q4_0: 67.6 -> 63.5; 16 rows, F16:
 // 67 -> 65.5).
 // All tiles of the call, rows in order, are dealt evenly to the CTAs and their warps, whatever the
-// lengths, beginning a unit counting for two tiles; a unit that falls to several warps is joined in shared memory, one that falls to
-// several CTAs through the workspace by the CTA that finishes last (partials in CTA order: the
-// same bits every time).
+// lengths, beginning a unit counting for two tiles; a unit that falls to several warps is joined in
+// shared memory, one that falls to several CTAs through the workspace by the CTA that finishes last
+// (partials in CTA order: the same bits every time).
 //
 // Measured (one B200, one layer, us a call, share of the measured HBM rate): 1 row over 131072
-// positions, 64 / 8 heads of 128, Q8_0: 66 (66 %); 64 rows over 512 to 16384 positions: 148 - 158
-// (74 - 79 %); 16 rows over 4096, BF16: 50 (82 %); 9 rows over 2048, 32 / 32 heads, Q4_0: 38 (30 %:
-// two columns of eight have work, and unpacking 4-bit codes for one query costs more cycles than
-// HBM takes). In cycles, the first: 2500 until every warp has its share, 6500 until it has asked
-// for its first four tiles, 15000 until the first product (queries and tiles arrive behind those of
-// 148 SMs), some 85000 of tiles, 8000 after the last (12 warps, then 18 CTAs are joined). 8-bit
-// codes as offset bytes took 70 more instructions a group for their conversion; 16 positions a tile
-// 78 us; queries held in registers before the first tile was asked for spilled.
+// positions, 64 / 8 heads of 128, Q8_0: 66 (66 %); 64 rows over 512 to 16384 positions: 150 - 161
+// (73 - 78 %); 16 rows over 4096, BF16: 50 (83 %); 9 rows over 2048, 32 / 32 heads, Q4_0: 38 - 39
+// (30 %: two columns of eight have work, and 8 warps an SM, each with one chain of scores, maximum,
+// weights and products a tile, issue in 38 % of the cycles). Rows of one sequence do not share its
+// cache: 128 rows of a prompt that end at position 4096, 64 / 8 heads: 201 (Q8_0), 266 (BF16), where
+// the bytes, read once, and the products are worth some 10. In cycles, the first: 2500 until every
+// warp has its share, 6500 until it has asked for its first four tiles, 15000 until the first product
+// (queries and tiles arrive behind those of 148 SMs), some 85000 of tiles, 8000 after the last (12
+// warps, then 18 CTAs are joined). 8-bit codes as offset bytes took 70 more instructions a group for
+// their conversion; 16 positions a tile 78 us; queries held in registers before the first tile was
+// asked for spilled. At heads of 128 and 8 queries, Q8_0, 12 warps leave 168 registers a thread, and
+// 84 bytes of them are spilled.
 //
 // Precision: results are f32. Cached values are exact in the fragments' type (codes of the 8- and
 // 4-bit types are small integers in f16, their scales are applied to scores and weights). The f32
 // operands are split: q (scaled per head by a power of two) and the weights (relative to the
-// tile's largest) into f16 hi + lo, 22 bits, or three bf16 parts, 24 bits, beside a bf16 cache.
-// f16 has the bits for weights within 2^24 of the tile's largest; smaller ones, which count where
-// a strong position's values are zero, go through the tensor cores in a pass of their own. The
-// tensor cores truncate when they add, so products accumulate over at most 32 dims or 32
-// positions there and are added up in f32 registers.
+// tile's largest) into f16 hi + lo, 22 bits, or three bf16 parts, 24 bits, beside a bf16 cache. The
+// f16 parts of a query end 2^-38 below the largest of its head, those of a weight 2^-38 below the
+// tile's largest; weights of fewer than 13 bits, which count where a strong position's values are
+// zero, and 8- and 4-bit caches' products of weights and V scales of fewer than 13 bits go through
+// the tensor cores in passes of their own (kSmall and kProd below). The tensor cores truncate when
+// they add, so products accumulate over at most 32 dims or 32 positions there and are added up in
+// f32 registers. Scores are f32 numbers; a key that is not finite gives NaN.
 #include <float.h>
 #include <limits.h>
 
@@ -456,7 +463,8 @@ template <int TYPE, int HD, bool PACK>
 __global__ void __launch_bounds__(PagedCfg<TYPE, HD, PACK>::THREADS, 1)
     k_paged_attn(const PagedAttnArgs a) {
     using C = PagedCfg<TYPE, HD, PACK>;
-    constexpr int X = C::X, W = C::W, NB = C::NB, NS = C::NS, NP = C::NP, HEADS = C::HEADS, S = C::S, NT = C::THREADS, TP = C::TP, TILE = C::TILE;
+    constexpr int X = C::X, W = C::W, NB = C::NB, NS = C::NS, NP = C::NP, HEADS = C::HEADS, S = C::S;
+    constexpr int NT = C::THREADS, TP = C::TP, TILE = C::TILE;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[W][S];
     __shared__ int s_red[3 * W];

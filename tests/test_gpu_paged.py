@@ -1104,3 +1104,36 @@ def test_the_largest_call_is_what_the_header_says(ctx):
                 kv.attention(q, none, table, out, work, seq=none, window=window)
                 assert (out == 0).all()
     kv.free()
+
+
+@pytest.mark.parametrize("wtype", TYPES)
+def test_a_chain_of_calls_under_programmatic_launch(ctx, wtype):
+    """Append, attention and read one after the other, each on what the one before wrote, many times
+    over: the bits of launches without it."""
+    rng = np.random.default_rng(31)
+    n, hk, h, d = 70, 2, 8, 64
+    x = torch.from_numpy(rng.standard_normal((n, (h + 2 * hk) * d)).astype(np.float32)).to(DEV)
+    table, work = i32([[4, 0, 2, 1, 3]]), None
+    got = []
+    try:
+        for on in (False, True):
+            ctx.set_pdl(on)
+            kv = ssdllm.PagedKvCache(ctx, 5, 16, hk, d, wtype)
+            work = kv.attention_workspace()
+            q, out, o = torch.empty(1, h * d, device=DEV), torch.zeros(n, h * d, device=DEV), torch.zeros(2, n, hk * d, device=DEV)
+            ints, seq = i32(np.arange(n + 1)), i32([0])
+            torch.cuda.synchronize()
+            for p in range(n):
+                at = ints[p:p + 1]
+                row = x[p:p + 1]
+                kv.append(row[:, h * d:(h + hk) * d], row[:, (h + hk) * d:], at, table, seq=seq, q=row[:, :h * d], q_out=q)
+                kv.attention(q, ints[p + 1:p + 2], table, out[p:p + 1], work, seq=seq)
+                kv.read(at, table, o[0, p:p + 1], o[1, p:p + 1], seq=seq)
+            torch.cuda.synchronize()
+            got.append((out, o))
+            kv.free()
+    finally:
+        ctx.set_pdl(False)
+    assert torch.isfinite(got[0][0]).all() and (got[0][1] != 0).any(-1).all()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
