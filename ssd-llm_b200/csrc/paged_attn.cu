@@ -33,8 +33,8 @@
 // (partials in CTA order: the same bits every time).
 //
 // Measured (one B200, one layer, us a call, share of the measured HBM rate): 1 row over 131072
-// positions, 64 / 8 heads of 128, Q8_0: 66 (66 %); 64 rows over 512 to 16384 positions: 150 - 161
-// (73 - 78 %); 16 rows over 4096, BF16: 50 (83 %); 9 rows over 2048, 32 / 32 heads, Q4_0: 38 - 39
+// positions, 64 / 8 heads of 128, Q8_0: 66 (66 %); 64 rows over 512 to 16384 positions: 148 - 161
+// (73 - 79 %); 16 rows over 4096, BF16: 50 (83 %); 9 rows over 2048, 32 / 32 heads, Q4_0: 38 - 39
 // (30 %: two columns of eight have work, and 8 warps an SM, each with one chain of scores, maximum,
 // weights and products a tile, issue in 38 % of the cycles). Rows of one sequence do not share its
 // cache: 128 rows of a prompt that end at position 4096, 64 / 8 heads: 201 (Q8_0), 266 (BF16), where
@@ -377,7 +377,7 @@ struct PagedGroup {
         uint32_t m = 0x7FFF7FFFu;
 #pragma unroll
         for (int b = 0; b < C::NB; b++) m = __vmins2(m, (vs[p * C::NB + b] & 0x7FFF7FFFu) + 0x7FFF7FFFu);
-        return (m & 0xFFFFu) - 0x7FFFu & 0xFFFFu | (m >> 16) - 0x7FFFu << 16;
+        return (((m & 0xFFFFu) - 0x7FFFu) & 0xFFFFu) | (((m >> 16) - 0x7FFFu) << 16);
     }
 };
 
